@@ -144,8 +144,10 @@ def _prepared(block_table, seq_lens, ref_counts, caches, parents):
 def _launch(name, block_table, seq_lens, ref_counts, caches, parents=None, with_map=False):
     caches, (p, _, pointers, scratch_bytes) = _prepared(block_table, seq_lens, ref_counts, caches, parents)
     device = block_table.device
-    # int32 rows without gaps like the arguments' own; torch.empty with a dtype and a device takes the host twice as long
-    new_table, new_refs = torch.empty_like(block_table), torch.empty_like(ref_counts)
+    # The kernels write rows without gaps.  empty_like would order the result's dimensions by the given table's strides,
+    # which need not be those of dense rows: rows of a table may overlap, as those of base.unfold(0, 4, 1) do.
+    # torch.empty with a dtype and a device takes the host twice as long.
+    new_table, new_refs = block_table.new_empty(block_table.shape), torch.empty_like(ref_counts)
     new_lens = torch.empty_like(seq_lens) if parents is not None else None
     page_map = torch.empty_like(ref_counts) if with_map else None
     count, scratch = block_table.new_empty(1), block_table.new_empty(scratch_bytes // 4)

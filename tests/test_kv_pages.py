@@ -351,3 +351,29 @@ def test_beam_search_over_a_4_bit_cache():
         for b in range(beams):
             write(whole, torch.arange(len(history[b])) + b * width * page, history[b])
         assert torch.equal(attend(cache, table, lens, q), attend(whole, plain.cuda(), lens, q))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 5])
+def test_tables_whose_rows_overlap(rows):
+    """Rows one element apart, fewer of them than columns and more: the result is dense whatever the table's strides."""
+    page, pool, width = 4, 40, 4
+    base = torch.randperm(pool, generator=torch.Generator().manual_seed(3)).to(torch.int32)[: rows + width - 1]
+    table = base.unfold(0, width, 1)
+    lens = np.array([14, 9, 16, 0, 3], np.int32)[:rows]
+    parents = np.array([0, 0, 1, 2, -1], np.int32)[:rows]
+    refs = np.zeros(pool, np.int32)
+    for b in range(rows):
+        np.add.at(refs, table[b, : -(-lens[b] // page)].numpy(), 1)
+    caches = _caches(pool, page, 0, ("odd",))
+    host = _host(caches)
+    on_device = base.cuda().unfold(0, width, 1)
+    assert on_device.stride() == (1, 1)
+    got = kv_pages.reassign_sequences(on_device, *_dev(lens, refs, parents), caches)
+    want = kv_pages_oracle.reassign(table.numpy().copy(), lens, refs, parents, host, page)
+    assert got[0].is_contiguous()
+    _check(got, (*want[:3], np.array([want[3]])), caches, host)
+    got = kv_pages.compact_pages(on_device, *_dev(lens, refs), caches)
+    want = kv_pages_oracle.compact(table.numpy().copy(), lens, refs, host, page)
+    assert got[0].is_contiguous()
+    _check(got, (*want[:3], np.array([want[3]])), caches, host)
