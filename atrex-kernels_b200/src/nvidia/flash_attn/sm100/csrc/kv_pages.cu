@@ -673,8 +673,10 @@ cudaError_t launch_one(const PageParams& k, const atrex_kvpages_sm100_params* p,
                          dim3(1 + (unsigned)std::min<long long>(std::max(std::max(copies, cells), 1ll), 2 * sms)),
                          dim3(kPlanThreads), sizeof(int) * p->num_pages, stream, k, caches, slices);
   const int meta = (int)std::min<long long>(std::max(cells, ((long long)p->num_pages + kPlanThreads - 1) / kPlanThreads) + 1, 16);
-  return launch_kernel(atrex_sm100_kvpages_compact_kernel<N>, dim3(meta + (unsigned)std::min<long long>(copies, 2 * sms - meta)),
-                       dim3(kPlanThreads), sizeof(uint16_t) * (2ull * p->num_pages + 2), stream, k, caches, slices, meta);
+  // all of the metadata CTAs, whose stride counts on each other, and one that copies at least, however few SMs are asked for
+  const long long copying = std::min<long long>(copies, std::max<long long>(1, 2ll * sms - meta));
+  return launch_kernel(atrex_sm100_kvpages_compact_kernel<N>, dim3((unsigned)(meta + copying)), dim3(kPlanThreads),
+                       sizeof(uint16_t) * (2ull * p->num_pages + 2), stream, k, caches, slices, meta);
 }
 
 // The second kernel over n caches from `done` on; the first such launch writes tables and counts too.

@@ -40,7 +40,8 @@ typedef struct atrex_kvpages_sm100_params {
   const atrex_kvpages_sm100_cache* caches;   /* HOST arrays of num_caches entries, read during the call: layouts */
   void* const* bases;                        /* and device addresses                                            */
   int64_t table_row_stride;
-  int32_t batch, width, num_pages, page_size, num_caches, sm_count;
+  int32_t batch, width, num_pages, page_size, num_caches;
+  int32_t sm_count;              /* SMs that the grids are sized for, 0 or less: all; results do not depend on it */
 } atrex_kvpages_sm100_params;
 
 ATREX_FA_API int atrex_kvpages_sm100_abi_version(void);

@@ -377,3 +377,37 @@ def test_tables_whose_rows_overlap(rows):
     want = kv_pages_oracle.compact(table.numpy().copy(), lens, refs, host, page)
     assert got[0].is_contiguous()
     _check(got, (*want[:3], np.array([want[3]])), caches, host)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sm_count", [1, 4, 8])
+@pytest.mark.parametrize("batch,page,width,pool", [(7, 4, 5, 60), (300, 2, 50, 1024), (300, 2, 50, 16384), (50, 2, 6, 16385)])
+def test_few_sms_through_the_c_abi(batch, page, width, pool, sm_count):
+    """The block's sm_count sizes the grids; whatever it says, every page and every entry of the tables is written."""
+    table, lens, refs = _state(batch, page, width, pool, 7)
+    parents = _parents(batch, 7)
+    caches = _caches(pool, page, 0, ("odd",))
+    host = _host(caches)
+    call = dict(zip(("block_table", "seq_lens", "ref_counts", "parents"), _dev(table, lens, refs, parents)))
+    for name in ("reassign", "compact"):
+        (block, _, pointers, scratch_bytes) = kv_pages._prepared(*list(call.values())[:3], caches, call["parents"])[1]
+        p = kv_pages.Params.from_buffer_copy(block)
+        bases = pointers(*[c.data_ptr() for c in caches])
+        p.bases, p.sm_count = ctypes.addressof(bases), sm_count
+        new = {f"new_{n}": torch.full_like(call[key], -9) for n, key in
+               (("table", "block_table"), ("lens", "seq_lens"), ("refs", "ref_counts"))}
+        new["page_map"], new["count"] = torch.full_like(call["ref_counts"], -9), torch.full_like(call["ref_counts"][:1], -9)
+        for field, tensor in (*call.items(), *new.items()):
+            setattr(p, field, tensor.data_ptr())
+        scratch = torch.empty(scratch_bytes, dtype=torch.uint8, device="cuda")
+        launch = getattr(kv_pages.library(), f"atrex_kvpages_sm100_{name}")
+        runtime.raise_for_status(launch(ctypes.byref(p), scratch.data_ptr(), scratch_bytes,
+                                        torch.cuda.current_stream().cuda_stream))
+        if name == "reassign":
+            want = kv_pages_oracle.reassign(table, lens, refs, parents, host, page)
+            _check((new["new_table"], new["new_lens"], new["new_refs"], new["count"]), (*want[:3], np.array([want[3]])),
+                   caches, host)
+        else:
+            want = kv_pages_oracle.compact(table, lens, refs, host, page)
+            _check((new["new_table"], new["new_refs"], new["page_map"], new["count"]), (*want[:3], np.array([want[3]])),
+                   caches, host)
