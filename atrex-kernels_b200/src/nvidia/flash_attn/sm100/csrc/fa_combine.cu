@@ -61,7 +61,9 @@ atrex_sm100_combine_kernel(const __grid_constant__ FwdParams p) {
     }
   }
   if (sink_l2 != -INFINITY) wsum += fast_exp2(sink_l2 - m_use);
-  const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
+  // Only a sum of nothing is "no key seen".  A split whose LSE is NaN (the query row is, or its scale) makes the sum NaN:
+  // output and LSE then say so, as they do without a split; -inf would give the row weight 0 in a later merge.
+  const float inv = wsum == 0.f ? 0.f : 1.f / wsum;
   __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + q_row * p.out_row_stride +
                        (int64_t)head * p.out_head_stride + lane * V;
 #pragma unroll
@@ -72,7 +74,7 @@ atrex_sm100_combine_kernel(const __grid_constant__ FwdParams p) {
     *reinterpret_cast<uint2*>(dst + i) = packed;
   }
   if (lane == 0 && p.lse != nullptr)
-    p.lse[(int64_t)head * p.total_q + q_row] = wsum > 0.f ? (m_use + log2f(wsum)) * kLn2 : -INFINITY;
+    p.lse[(int64_t)head * p.total_q + q_row] = wsum == 0.f ? -INFINITY : (m_use + log2f(wsum)) * kLn2;
 }
 
 constexpr int kPlanThreads = 1024;

@@ -681,3 +681,27 @@ def test_pools_beyond_4_gb(monkeypatch):
     for b, i, src in ((0, 0, 0), (0, 3, 3), (0, 4, 4), (2, 0, 6), (2, 1, 9)):
         for a, c in zip(near, far):
             assert torch.equal(c[int(rows[b, i])].view(torch.uint8), a[src].view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits", [1, 2, 5, 9, 16])
+@pytest.mark.parametrize("q_lens", [[1, 1, 1], [6, 0, 4], [130, 1, 20]])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_the_lse_of_a_nan_query_row_is_nan(q_lens, splits, sinks, route):
+    """However the splits join (in the kernel, over a cluster, through scratch): -inf would mean that no key was seen,
+    and give the row weight 0 in a merge.  A row of NaN that sees no key is still empty."""
+    c = make_case(q_lens, [700, 30, 500], 8, 2, 128, 64, seed=6, sinks=sinks)
+    args = gpu_args(c, num_splits=splits)
+    head = 5
+    args["q"] = args["q"].clone()
+    args["q"][:, head] = float("nan")
+    out, lse = atrex.flash_attn_varlen_func(**args)
+    assert out[:, head].isnan().all() and lse[head].isnan().all()
+    others = [h for h in range(8) if h != head]
+    assert out[:, others].isfinite().all() and lse[others].isfinite().all()
+    args["seqused_k"].zero_()
+    out, lse = atrex.flash_attn_varlen_func(**args)
+    assert not out.any()
+    want = args["s_aux"].float()[:, None].expand_as(lse) if sinks else torch.full_like(lse, -float("inf"))
+    # |sink| log2 e + 7 stays below 16, where a rounding is off by 2^-21; the exponential and the products by 2^-22 relative
+    assert torch.allclose(lse, want, rtol=2.0 ** -20, atol=2.0 ** -20)
