@@ -24,7 +24,7 @@
 // Measured (32 / 8 heads of 128): one request of 4 097 keys 10.4 us; 64 requests of 1 024 .. 16 384 keys 144 us = 4.1 TB/s
 // of codes and scales, 91 us at the measured copy rate; 300 of 1 000 keys 92 us (53).  What bounds it: instruction issue.
 // A token and head costs ~19 warp instructions, of which 12 widen (convert, multiply by the block scale); three warps per
-// scheduler, which is what 160 registers allow, issue in 0.6 of the cycles (math pipes busy and fixed latencies).  Four
+// scheduler, which is what 162 registers allow, issue in 0.6 of the cycles (math pipes busy and fixed latencies).  Four
 // CTAs per SM in 128 registers: 158 us.  Codes by TMA: 154 against 144 (one lane's issue and polling cost more than eight
 // cp.async a lane).  A CTA costs ~3.5 us besides its tiles, hence few splits (the rule is the launcher's).  Warps with
 // equal shares of all tiles of the call: 138 us here, but 300 requests of 100 .. 4 000 keys 172 -> 188.
@@ -132,6 +132,12 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 2 ? 3 : 1) atrex_sm100_kv4_
   int kv_end = kv_len, kv_begin = 0;
   if (p.window_right >= 0) kv_end = min(kv_len, right_bound(p, qi_hi + off));
   if (p.window_left >= 0) kv_begin = max(0, qi_lo + off - p.window_left);
+  // keys lo .. hi - 1 that packed row r of this CTA sees
+  auto row_keys = [&](int r, int& lo, int& hi) {
+    const int qi = min((row0 + r) / p.group, q_len - 1);
+    hi = p.window_right >= 0 ? min(kv_len, right_bound(p, qi + off)) : kv_len;
+    lo = p.window_left >= 0 ? max(0, qi + off - p.window_left) : 0;
+  };
   // keys every row of this CTA sees
   const int full_lo = p.window_left >= 0 ? max(0, qi_hi + off - p.window_left) : 0;
   const int full_hi = p.window_right >= 0 ? min(kv_len, right_bound(p, qi_lo + off)) : kv_len;
@@ -291,8 +297,12 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 2 ? 3 : 1) atrex_sm100_kv4_
             qf[nb][c][2 * u + (i >> 1)][i & 1] =
                 pack_f16(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up);
         }
-      factor[nb][0] = score_factor(__shfl_sync(0xffffffffu, down, 8 * t) * scale_log2);
-      factor[nb][1] = score_factor(__shfl_sync(0xffffffffu, down, 8 * t + 4) * scale_log2);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        int lo, hi;
+        row_keys(nb * 8 + 2 * t + i, lo, hi);
+        factor[nb][i] = score_factor(__shfl_sync(0xffffffffu, down, 8 * t + 4 * i) * scale_log2, lo < hi);
+      }
     }
   }
 
@@ -376,11 +386,7 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 2 ? 3 : 1) atrex_sm100_kv4_
       if (need_mask) {
         int lo[2], hi[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int qi = min((row0 + nb * 8 + 2 * t + i) / p.group, q_len - 1);
-          hi[i] = p.window_right >= 0 ? min(kv_len, right_bound(p, qi + off)) : kv_len;
-          lo[i] = p.window_left >= 0 ? max(0, qi + off - p.window_left) : 0;
-        }
+        for (int i = 0; i < 2; ++i) row_keys(nb * 8 + 2 * t + i, lo[i], hi[i]);
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll

@@ -506,7 +506,6 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
       if (!it.valid) break;
       const int sub_row0 = it.row0 + w * kBM;
       const int n_tiles = it.n_tiles, tile_lo = it.tile_lo;
-      const float scale_log2 = score_factor(it.scale_log2 * row_factor[(n_item & 1u) * kRowsPerItem + w * kBM + r]);
       int vis_lo, vis_hi, full_lo, full_hi;
       {
         const int q_last = max(it.q_len - 1, 0), off = it.off, kv_len = it.kv_len;
@@ -517,6 +516,8 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
         full_lo = p.window_left >= 0 ? max(0, sqi_hi + off - p.window_left) : 0;
         full_hi = p.window_right >= 0 ? min(kv_len, right_bound(p, sqi_lo + off)) : kv_len;
       }
+      const float scale_log2 =
+          score_factor(it.scale_log2 * row_factor[(n_item & 1u) * kRowsPerItem + w * kBM + r], vis_lo < vis_hi);
       bool dead = false;
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = 0; j < n_tiles; ++j) {

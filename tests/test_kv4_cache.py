@@ -705,3 +705,35 @@ def test_the_lse_of_a_nan_query_row_is_nan(q_lens, splits, sinks, route):
     want = args["s_aux"].float()[:, None].expand_as(lse) if sinks else torch.full_like(lse, -float("inf"))
     # |sink| log2 e + 7 stays below 16, where a rounding is off by 2^-21; the exponential and the products by 2^-22 relative
     assert torch.allclose(lse, want, rtol=2.0 ** -20, atol=2.0 ** -20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits", [0, 1, 3])
+@pytest.mark.parametrize("q_lens,d", [([1, 1, 1], 128), ([2, 9, 1], 256), ([1, 40, 150], 128)])
+def test_factors_of_either_sign_and_zero(q_lens, d, splits, route):
+    c = make_case(q_lens, [700, 30, 90], 8, 2, d, 64, seed=15, factors=True, sinks=True)
+    c["kf"], c["vf"] = c["kf"] * torch.tensor([[1.0, -1], [-1, 0], [-1, 1]]), c["vf"] * torch.tensor([[-1.0, 1], [0, 1], [-1, -1]])
+    out, lse = atrex.flash_attn_varlen_func(**gpu_args(c, num_splits=splits))
+    check(c, out, lse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("splits", [0, 1, 3, 9])
+@pytest.mark.parametrize("q_lens,d", [([1, 1, 1], 128), ([2, 50, 1], 256), ([1, 40, 150], 128)])
+def test_a_nan_factor_shows(q_lens, d, splits, route):
+    """A NaN k_descale of one KV head: its rows are NaN if they see a key and empty if they see none; the others keep
+    their bits."""
+    c = make_case(q_lens, [700, 30, 90], 8, 2, d, 64, seed=16, factors=True)
+    args = gpu_args(c, num_splits=splits)
+    out, lse = atrex.flash_attn_varlen_func(**args)
+    check(c, out, lse)
+    args["k_descale"] = args["k_descale"].clone()
+    args["k_descale"][1:, 1] = float("nan")
+    got, got_lse = atrex.flash_attn_varlen_func(**args)
+    rows, other = slice(q_lens[0], None), slice(0, q_lens[0])
+    assert torch.equal(got[:, :4], out[:, :4]) and torch.equal(got_lse[:4], lse[:4])
+    assert torch.equal(got[other], out[other]) and torch.equal(got_lse[:, other], lse[:, other])
+    sees = ~lse[4:, rows].isneginf()
+    assert got_lse[4:, rows][sees].isnan().all() and got[rows, 4:].transpose(0, 1)[sees].isnan().all()
+    assert got_lse[4:, rows][~sees].isneginf().all() and not got[rows, 4:].transpose(0, 1)[~sees].any()
+    assert bool((~sees).any()) == (q_lens[1] > 30)
