@@ -153,12 +153,24 @@ int resolve(const atrex_kv4_sm100_params* pp, int sm_count, Resolved* r) {
   const int64_t tile = prefill ? kv4_prefill_tile(p->head_dim) : 32, most = (span + tile - 1) / tile;
   int64_t splits = r->kernel == kDouble ? 1 : p->num_splits;
   if (splits == 0 && prefill) {
-    // Items walk the SMs in rounds; an item costs about four tiles besides its own (Q rows, first scores, epilogue),
-    // and partial results as much again.  `items` counts whole requests' tiles and is an upper bound when tiled.
-    int64_t best = -1;
-    for (int64_t s = 1; s <= most && s <= 64; ++s) {
-      const int64_t cost = ((items * s + sm_count - 1) / sm_count) * ((most + s - 1) / s + 4) + (s > 1 ? 4 : 0);
-      if (best < 0 || cost < best) {
+    // Items walk the SMs in rounds; an item costs about four tiles besides its own (Q rows, first scores, epilogue).
+    // A split call pays for its partial results: the combine kernel as much again and about a tile per split (it reads
+    // them one after the other), and their bytes, of which 4 MB written and read take a tile's 1.3 us.  `items` is an
+    // upper bound when tiled and lengths vary, so only a gain of more than a sixteenth counts; beyond four rounds nothing
+    // is split, nor into more than 256 MB of partial results.  Microseconds by splits, head_dim 256 (requests, heads,
+    // query tokens, longest context):
+    //   15, 64 / 4, 1 .. 27, 12 406: 1: 242, 3: 160, 5: 165, 7: 169;  1, 64 / 4, 5, window 4 129: 8: 21, 16: 30, 34: 39
+    //   16, 24 / 2, 1 .. 96, 8 192: 1: 185, 2: 160, 4: 157, 5: 171;   59, 12 / 1, 10 .. 27, 2 027: 1: 65, 2: 80
+    //   1, 64 / 8, 512, 16 384: 1: 680, 2: 734, 5: 751;   3, 32 / 8, 900 .. 1 060, 12 974: 1: 1 073, 2: 1 144, 3: 1 171
+    const int64_t part = 4 * (int64_t)p->total_q * p->num_q_heads * (p->head_dim + 1);     // bytes of a split's results
+    int64_t unsplit = 0, best = 0;
+    splits = 1;
+    for (int64_t s = 1; s <= most && s <= 64 && (s == 1 || items <= 4 * (int64_t)sm_count); ++s) {
+      int64_t cost = ((items * s + sm_count - 1) / sm_count) * ((most + s - 1) / s + 4);
+      if (s > 1 && s * part > (256 << 20)) break;
+      if (s > 1) cost += 4 + s + s * part / (4 << 20);
+      if (s == 1) unsplit = best = cost;
+      if (cost < best && cost * 16 < unsplit * 15) {
         best = cost;
         splits = s;
       }

@@ -231,6 +231,41 @@ def test_native_plan():
     assert kv4.library().atrex_kv4_sm100_write(None, None) == 1
 
 
+def _prompt_plan(batch, max_q, total_q, hq, hkv, d, max_k, window=-1, route=2):
+    rows = {f"{side}_{kind}row_stride": d // w for side in "kv" for kind, w in (("", 2), ("scale_", 16))}
+    status, info = _plan_status(batch=batch, max_seqlen_q=max_q, total_q=total_q, num_q_heads=hq, num_kv_heads=hkv,
+                                head_dim=d, max_seqlen_k=max_k, window_left=window, route=route,
+                                max_pages_per_seq=-(-max_k // 64), **rows)
+    assert status == 0
+    return info
+
+
+def test_long_prompts_are_not_split():
+    """Splits that save a fraction of a round of work do not pay for the partial results they leave in scratch."""
+    for batch, max_q, total_q, hq, hkv, max_k in ((4, 9984, 39936, 64, 8, 131072), (3, 1060, 2940, 32, 8, 12974),
+                                                  (26, 1148, 11648, 24, 2, 45081), (309, 61, 6798, 64, 4, 93574)):
+        info = _prompt_plan(batch, max_q, total_q, hq, hkv, 256, max_k)
+        assert info.num_splits == 1 and info.workspace_bytes < 4096
+    # few row tiles over a long context are split, in as many parts as the combine kernel joins in a few microseconds
+    for batch, max_q, total_q, hq, hkv, d, max_k, window in ((1, 16, 16, 16, 2, 256, 8192, -1), (1, 5, 4, 64, 4, 256, 14372, 4129),
+                                                             (2, 100, 200, 8, 2, 256, 10000, -1), (8, 5, 40, 64, 4, 128, 8192, -1)):
+        assert 2 <= _prompt_plan(batch, max_q, total_q, hq, hkv, d, max_k, window).num_splits <= 16
+
+
+def test_scratch_of_automatic_splits_is_bounded():
+    """At most four rounds of 128-row items are split, and only where their partial results cost less than they gain."""
+    r = np.random.RandomState(4)
+    heads = ((32, 8), (64, 8), (64, 4), (24, 2), (16, 2), (8, 1), (12, 1), (64, 1))
+    for _ in range(4000):
+        hq, hkv = heads[r.randint(len(heads))]
+        batch, max_q, max_k = (int(2 ** r.uniform(0, top)) for top in (9, 13, 18))
+        d, total_q = int(r.choice([128, 256])), batch * int(r.randint(1, max_q + 1))
+        info = _prompt_plan(batch, max_q, total_q, hq, hkv, d, max_k, int(r.choice([-1, 1000])))
+        assert info.workspace_bytes <= 2 ** 28 + 16 * batch + 1024       # partial results, and the plan of the row tiles
+        if info.num_splits > 1:
+            assert total_q * hq <= 4 * 148 * 128
+
+
 # ------------------------------------------------------------------ GPU: the write
 def _pool(layout, pages, page, heads, dim, fill=0xA5):
     """(codes, scales) in one of the layouts the attention call accepts, every byte ``fill``."""
