@@ -188,9 +188,12 @@ int resolve(const atrex_kv4_sm100_params* pp, int sm_count, Resolved* r) {
   if (splits > kMaxSplits) splits = kMaxSplits;
   if (splits < 1) splits = 1;
   r->splits = (int)splits;
-  // Splits join inside the decode kernel while the whole call is one wave of CTAs (four fit an SM); in larger calls
-  // clusters, which start together, cost more than the combine kernel (decode of 64 requests, 4 splits: 161 against 151 us).
-  r->parts = splits > 1 && !(r->kernel == kDecode && splits <= kv4_decode_max_cluster() && items * splits <= 4ll * sm_count);
+  // Splits join inside the decode kernel while the whole call is one wave of CTAs; in larger calls clusters, which start
+  // together, cost more than the combine kernel.  Microseconds, cluster / combine: 64 requests of 1 024 .. 16 384 keys,
+  // 2 048 CTAs: 161 / 151; 512 CTAs at head_dim 128: 49.6 / 47.7, 55.8 / 49.5, 33.3 / 31.4; 320 and 400 at 256: 47.6 / 43.4,
+  // 73.5 / 66.5.  Within a wave the cluster wins: one request of 4 097 keys 14.5 -> 12.5 (the kernel's first version).
+  const int64_t wave = (int64_t)kv4_decode_resident(p->head_dim) * sm_count;
+  r->parts = splits > 1 && !(r->kernel == kDecode && splits <= kv4_decode_max_cluster() && items * splits <= wave);
   uint64_t off = 0;
   r->off_order = off;
   if (r->tiled) off = align_up(off + 4ull * p->batch, 256);

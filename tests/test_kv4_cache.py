@@ -231,6 +231,17 @@ def test_native_plan():
     assert kv4.library().atrex_kv4_sm100_write(None, None) == 1
 
 
+@pytest.mark.parametrize("d,resident", [(128, 3), (256, 2)])
+def test_splits_join_in_the_kernel_within_one_wave(d, resident):
+    """... of the CTAs that fit the SMs (by registers: three and two an SM); beyond it through scratch."""
+    rows = {f"{side}_{kind}row_stride": d // w for side in "kv" for kind, w in (("", 2), ("scale_", 16))}
+    wave = resident * 148
+    for batch, splits in ((wave // 4, 4), (wave // 4 + 1, 4), (wave // 8, 8), (wave // 8 + 1, 8), (wave // 2 + 1, 2), (148, 4)):
+        status, info = _plan_status(batch=batch, total_q=batch, num_q_heads=4, num_kv_heads=1, head_dim=d, num_splits=splits, **rows)
+        assert status == 0 and info.num_splits == splits
+        assert info.kernel_launches == (1 if batch * splits <= wave else 2)
+
+
 def _prompt_plan(batch, max_q, total_q, hq, hkv, d, max_k, window=-1, route=2):
     rows = {f"{side}_{kind}row_stride": d // w for side in "kv" for kind, w in (("", 2), ("scale_", 16))}
     status, info = _plan_status(batch=batch, max_seqlen_q=max_q, total_q=total_q, num_q_heads=hq, num_kv_heads=hkv,
