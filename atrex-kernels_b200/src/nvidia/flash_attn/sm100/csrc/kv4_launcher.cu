@@ -37,6 +37,58 @@ bool strides_small(std::initializer_list<int64_t> strides) {
   return true;
 }
 
+// Rows of `bytes` bytes, tokens x heads of them, at byte strides.
+struct Rows {
+  const void* base;
+  int64_t token, head;
+};
+bool same_rows(const Rows& a, const Rows& b) { return a.base == b.base && a.token == b.token && a.head == b.head; }
+// Whether a row of `a` and a row of `b` share a byte; with `a` itself for `b`: two different rows of it.  Two sets of
+// unlike strides that lie within each other's range count as sharing.
+bool rows_meet(const Rows& a, const Rows& b, int64_t tokens, int64_t heads, int64_t bytes) {
+  const bool self = same_rows(a, b);
+  const int64_t first_a = (int64_t)reinterpret_cast<intptr_t>(a.base), first_b = (int64_t)reinterpret_cast<intptr_t>(b.base);
+  const int64_t last_a = first_a + (tokens - 1) * a.token + (heads - 1) * a.head + bytes;
+  const int64_t last_b = first_b + (tokens - 1) * b.token + (heads - 1) * b.head + bytes;
+  if (last_a <= first_b || last_b <= first_a) return false;
+  if (a.token != b.token || a.head != b.head) return true;
+  // equal strides: some row of b is dt tokens and dh heads away and less than a row's bytes
+  for (int64_t dh = 1 - heads; dh < heads; ++dh) {
+    const int64_t apart = first_b - first_a + dh * a.head;
+    if (a.token == 0) {
+      if (apart < bytes && -apart < bytes && !(self && dh == 0 && tokens == 1)) return true;
+      continue;
+    }
+    const int64_t floor = apart >= 0 ? apart / a.token : -((-apart + a.token - 1) / a.token);
+    for (int64_t back = floor; back <= floor + 1; ++back) {         // the two nearest
+      const int64_t dt = std::max(1 - tokens, std::min(tokens - 1, back));
+      const int64_t gap = apart - dt * a.token;
+      if (gap < bytes && -gap < bytes && !(self && dh == 0 && dt == 0)) return true;
+    }
+  }
+  return false;
+}
+
+// The out rows are written while other CTAs still read key and value and write the other side's rows.
+bool outs_alias(const atrex_kv4_sm100_write_params* p) {
+  auto rows = [&](const void* base, int64_t token, int64_t head) -> Rows {      // strides of single tokens and heads say nothing
+    return {base, p->num_tokens > 1 ? 2 * token : 0, p->num_kv_heads > 1 ? 2 * head : 0};
+  };
+  const Rows in[2] = {rows(p->key, p->key_token_stride, p->key_head_stride),
+                      rows(p->value, p->value_token_stride, p->value_head_stride)};
+  const Rows out[2] = {rows(p->key_out, p->key_out_token_stride, p->key_out_head_stride),
+                       rows(p->value_out, p->value_out_token_stride, p->value_out_head_stride)};
+  auto meet = [&](const Rows& a, const Rows& b) { return rows_meet(a, b, p->num_tokens, p->num_kv_heads, 2ll * p->head_dim); };
+  for (int i = 0; i < 2; ++i) {
+    if (out[i].base == nullptr) continue;
+    if (meet(out[i], out[i])) return true;                          // of an expanded tensor, say
+    if (!same_rows(out[i], in[i]) && meet(out[i], in[i])) return true;
+    // a set of rows and itself have no two rows that meet, but here the two are written and read as one
+    if (same_rows(out[i], in[1 - i]) || meet(out[i], in[1 - i])) return true;
+  }
+  return out[0].base != nullptr && out[1].base != nullptr && (same_rows(out[0], out[1]) || meet(out[0], out[1]));
+}
+
 int check_write(const atrex_kv4_sm100_write_params* p) {
   if (p == nullptr) return report_failure(ATREX_FA_INVALID_VALUE, "parameter block is NULL");
   if (p->struct_bytes != sizeof(*p) || p->abi_version != ATREX_KV4_SM100_ABI_VERSION)
@@ -56,6 +108,9 @@ int check_write(const atrex_kv4_sm100_write_params* p) {
       (p->key_out && !strides_ok({p->key_out_token_stride, p->key_out_head_stride}, 2, 32)) ||
       (p->value_out && !strides_ok({p->value_out_token_stride, p->value_out_head_stride}, 2, 32)))
     return report_failure(ATREX_FA_UNSUPPORTED, "key / value / key_out / value_out rows must start on 32-byte boundaries");
+  if (outs_alias(p))
+    return report_failure(ATREX_FA_INVALID_VALUE, "key_out / value_out may be key / value themselves, but must not overlap "
+                                                  "them, each other or themselves in any other way");
   if (!aligned(p->key_cache, 8) || !aligned(p->value_cache, 8) ||
       !strides_ok({p->key_cache_page_stride, p->key_cache_row_stride, p->key_cache_head_stride,
                    p->value_cache_page_stride, p->value_cache_row_stride, p->value_cache_head_stride}, 1, 8) ||

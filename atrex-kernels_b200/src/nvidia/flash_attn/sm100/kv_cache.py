@@ -109,7 +109,8 @@ def write_kv_cache(key, value, key_cache, value_cache, slot_mapping, k_scale=Non
     4-bit caches (uint8) take their ``key_block_scale`` / ``value_block_scale`` tensors along.  ``key_out`` /
     ``value_out`` (BF16 like ``key``; may be ``key`` / ``value`` themselves) then receive the rows as the cache holds
     them, ``bf16(code * scale * factor)``, so that a prompt's own attention can see what later steps will read; rows
-    of skipped tokens are left as they were."""
+    of skipped tokens are left as they were.  In any other way they must not overlap ``key``, ``value``, each other or
+    themselves (``ValueError``): where ``key`` and ``value`` are one tensor, ``key_out`` is another."""
     if key_cache.dtype == torch.uint8 or key_block_scale is not None or value_block_scale is not None:
         return kv4.write(key, value, key_cache, value_cache, key_block_scale, value_block_scale, slot_mapping, k_scale,
                          v_scale, key_out, value_out)

@@ -29,7 +29,9 @@ extern "C" {
  * is not kept.  A factor is positive, between 2^-100 and 2^100.  Slots are distinct: of tokens with one slot any mixture
  * may be kept.
  * key_out / value_out (NULL, or BF16 like key with strides of their own) receive the stored rows,
- * bf16(code * step); rows of skipped tokens are left as they were.
+ * bf16(code * step); rows of skipped tokens are left as they were.  key_out may be key and value_out value (the same
+ * address and strides); otherwise rows of key_out and value_out share no byte with key, value or another row of either
+ * (ATREX_FA_INVALID_VALUE; tensors of unlike strides whose address ranges meet are taken to share one).
  * Strides are in elements of their tensor (bytes for the caches).  head_dim is a multiple of 16; key, value and the
  * out rows start on 32-byte boundaries (base and strides), code rows on 8-byte ones.
  */

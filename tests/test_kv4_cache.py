@@ -231,6 +231,60 @@ def test_native_plan():
     assert kv4.library().atrex_kv4_sm100_write(None, None) == 1
 
 
+def _write_status(tokens, heads, dim, **rows):
+    """Status of the C entry for rows given as (address, token stride, head stride); 0 or a CUDA error without a device."""
+    p = kv4.WriteParams()
+    p.struct_bytes, p.abi_version = ctypes.sizeof(p), kv4.ABI_VERSION
+    p.num_tokens, p.num_kv_heads, p.head_dim, p.page_size, p.num_pages = tokens, heads, dim, 16, 0
+    p.slot_mapping = 4096
+    for name, (base, token, head) in rows.items():
+        setattr(p, name, base)
+        setattr(p, f"{name}_token_stride", token)
+        setattr(p, f"{name}_head_stride", head)
+    return kv4.library().atrex_kv4_sm100_write(ctypes.byref(p), None)
+
+
+def test_out_rows_that_overlap_are_refused(monkeypatch):
+    """Against the bytes of every row, one by one.  No pool is behind the calls and no device here: a call that passes
+    the checks ends at the device's."""
+    if torch.cuda.is_available():
+        pytest.skip("addresses are made up")
+    r = np.random.RandomState(0)
+    dim, refused, accepted = 16, 0, 0
+
+    def taken(rows, tokens, heads):
+        base, token, head = rows
+        return [{base + 2 * (t * token + h * head) + b for b in range(2 * dim)} for t in range(tokens) for h in range(heads)]
+
+    for _ in range(1500):
+        tokens, heads = int(r.randint(1, 5)), int(r.randint(1, 4))
+        strides = [(int(a), int(b)) for a, b in ((heads * dim, dim), (3 * heads * dim, dim), (dim, tokens * dim), (0, dim),
+                                                 (heads * dim, 0), (48, 16), (32, 48))]
+        strides = strides[r.randint(0, 4 if r.rand() < 0.7 else len(strides))]
+        key, value = [(1 << 20) + 32 * int(r.randint(0, 30)) for _ in range(2)]
+        rows = {"key": (key, *strides), "value": (value if r.rand() < 0.8 else key, *strides)}
+        for name, own in (("key_out", key), ("value_out", value)):
+            if r.rand() < 0.7:
+                rows[name] = (own if r.rand() < 0.5 else (1 << 20) + 32 * int(r.randint(0, 60)), *strides)
+        bad, sets = False, {name: taken(at, tokens, heads) for name, at in rows.items()}
+        for out, own in (("key_out", "key"), ("value_out", "value")):
+            if out not in rows:
+                continue
+            bad |= len(set().union(*sets[out])) < 2 * dim * tokens * heads
+            for name in rows:
+                if name != out and not (name == own and rows[name] == rows[out]):
+                    bad |= bool(set().union(*sets[out]) & set().union(*sets[name]))
+        assert (_write_status(tokens, heads, dim, **rows) == 1) == bad, (tokens, heads, rows)
+        refused, accepted = refused + bad, accepted + (not bad)
+    assert min(refused, accepted) > 300
+    # rows of a fused QKV tensor lie between each other; other strides in the same range are refused, outside it are not
+    fused = {"key": (4096, 384, 16), "value": (4096 + 2 * 128, 384, 16)}
+    assert _write_status(9, 8, 16, key_out=fused["key"], value_out=fused["value"], **fused) != 1
+    assert _write_status(9, 8, 16, key_out=(4096 + 2 * 256, 400, 16), **fused) == 1
+    assert _write_status(9, 8, 16, key_out=(1 << 20, 128, 16), **fused) != 1
+    assert _write_status(1, 8, 16, key_out=(4096, 128, 16), **fused) != 1        # one token: its stride says nothing
+
+
 @pytest.mark.parametrize("d,resident", [(128, 3), (256, 2)])
 def test_splits_join_in_the_kernel_within_one_wave(d, resident):
     """... of the CTAs that fit the SMs (by registers: three and two an SM); beyond it through scratch."""
@@ -783,3 +837,21 @@ def test_a_nan_factor_shows(q_lens, d, splits, route):
     assert got_lse[4:, rows][sees].isnan().all() and got[rows, 4:].transpose(0, 1)[sees].isnan().all()
     assert got_lse[4:, rows][~sees].isneginf().all() and not got[rows, 4:].transpose(0, 1)[~sees].any()
     assert bool((~sees).any()) == (q_lens[1] > 30)
+
+
+@pytest.mark.gpu
+def test_write_refuses_outs_that_overlap_its_inputs():
+    heads, dim, tokens, page = 4, 128, 40, 16
+    k, ks, v, vs = kv_cache.allocate_fp4_kv_cache(4, page, heads, dim)
+    store = _rows(tokens + 1, heads, dim, 3, False).cuda()
+    rows, shifted, other = store[:-1], store[1:], torch.zeros_like(store[:-1])
+    slots, before = torch.arange(tokens, device="cuda"), store.clone()
+    for outs in (dict(key_out=rows), dict(value_out=rows), dict(key_out=other, value_out=other), dict(key_out=shifted),
+                 dict(value_out=other[:1].expand_as(rows))):
+        with pytest.raises(ValueError, match="overlap"):
+            kv_cache.write_kv_cache(rows, rows, k, v, slots, key_block_scale=ks, value_block_scale=vs, **outs)
+    torch.cuda.synchronize()
+    assert torch.equal(store, before) and not k.any() and not v.any()
+    kv_cache.write_kv_cache(rows, rows, k, v, slots, key_block_scale=ks, value_block_scale=vs, key_out=other)
+    want = torch.from_numpy(kv4_oracle.quantise(rows.float().cpu().numpy())[2]).float().bfloat16()
+    assert torch.equal(other.cpu(), want) and torch.equal(store, before) and torch.equal(k, v)
