@@ -187,20 +187,22 @@ __device__ __forceinline__ void widen_row(const uint8_t* stage, uint8_t* tile, i
   }
 }
 
-// A bounded wait: on expiry one lane reports and the warp leaves its loop.
-#define KV4_WAIT_OR_LEAVE(ok, code)                               \
-  if (!(ok)) {                                                    \
-    if (lane == 0) {                                              \
-      if (p.status) atomicExch(p.status, (code));                 \
-      atomicExch(abort_flag, 1);                                  \
-    }                                                             \
-    break;                                                        \
+// A bounded wait that expired: one lane reports.
+#define KV4_REPORT(code)                              \
+  if (lane == 0) {                                    \
+    if (p.status) atomicExch(p.status, (code));       \
+    atomicExch(abort_flag, 1);                        \
   }
-// A warp goes on or gives up as one where TMEM accesses or warp barriers behind the wait need all of its lanes.
-#define KV4_WAIT(bar_index, parity, code) \
-  KV4_WAIT_OR_LEAVE(__all_sync(0xffffffffu, mbar_wait(&bars[bar_index], (parity))), code)
-// Issuer, producers (votes in their chains: 1 930 -> 2 000 us for the chunk case) and the item warp's one lane.
-#define KV4_LANE_WAIT(bar_index, parity, code) KV4_WAIT_OR_LEAVE(mbar_wait(&bars[bar_index], (parity)), code)
+// A warp goes on or leaves its loop as one: TMEM accesses and warp barriers behind a wait need all of its lanes.  The tile
+// loops of issuer and producers hold neither, because a vote there costs (chunk case, us: 1 830; at every wait 1 900, in
+// place of the producers' barrier behind a stage 1 885): their lanes give up one by one and the warp votes once an item.
+#define KV4_WAIT(bar_index, parity, code)                                          \
+  if (!__all_sync(0xffffffffu, mbar_wait(&bars[bar_index], (parity)))) {           \
+    KV4_REPORT(code)                                                               \
+    break;                                                                         \
+  }
+#define KV4_LANE_WAIT(bar_index, parity) \
+  if (!mbar_wait(&bars[bar_index], (parity))) break;
 
 __global__ void __launch_bounds__(kThreads, 1)
 atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
@@ -316,7 +318,10 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
         uint32_t n = 0;
         for (int item = blockIdx.x;; item += gridDim.x, ++n) {
           Item* slot = slots + (n & 1u);
-          if (n >= 2) KV4_LANE_WAIT(kItemEmpty + (n & 1u), ((n >> 1) - 1u) & 1u, kWaitEmptyTimeout)
+          if (n >= 2 && !mbar_wait(&bars[kItemEmpty + (n & 1u)], ((n >> 1) - 1u) & 1u)) {
+            KV4_REPORT(kWaitEmptyTimeout)
+            break;
+          }
           resolve_item(p, item, *slot);
           if (*(volatile int*)abort_flag) slot->valid = 0;
           const bool valid = slot->valid != 0;
@@ -334,7 +339,7 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
       const int box_rows = p.box_rows;
       uint32_t n = 0;                                  // tiles of the run: K even, V odd
       for (uint32_t n_item = 0;; ++n_item) {
-        KV4_LANE_WAIT(kItemFull + (n_item & 1u), (n_item >> 1) & 1u, kWaitFullTimeout)
+        KV4_WAIT(kItemFull + (n_item & 1u), (n_item >> 1) & 1u, kWaitFullTimeout)
         const Item& it = slots[n_item & 1u];
         if (!it.valid) break;
         const int kv_begin = it.kv_begin, kv_end = it.kv_end, n_tiles = it.n_tiles, kvh = it.kvh;
@@ -363,7 +368,7 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
           for (int v = 0; v < 2; ++v, ++n) {
             const uint32_t stage = n % kStages;
             dead = true;
-            if (n >= (uint32_t)kStages) KV4_LANE_WAIT(kStageEmpty + stage, ((n / kStages) - 1u) & 1u, kWaitEmptyTimeout)
+            if (n >= (uint32_t)kStages) KV4_LANE_WAIT(kStageEmpty + stage, ((n / kStages) - 1u) & 1u)
             dead = false;
             uint8_t* dst = stage_smem + stage * kStageBytes;
             uint64_t* full = &bars[kStageFull + stage];
@@ -395,13 +400,15 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
               }
               asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full)) : "memory");
             }
-            __syncwarp();
           }
           if (dead) break;
 #pragma unroll
           for (int u = 0; u < 4; ++u) page[u] = next[u];
         }
-        if (dead) break;
+        if (__any_sync(0xffffffffu, dead)) {
+          KV4_REPORT(kWaitEmptyTimeout)
+          break;
+        }
       }
       // every copy must have landed before the CTA may exit
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -430,19 +437,19 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
         umma_commit_lead(lead, &bars[kSFull + w]);
       };
       for (uint32_t n_item = 0;; ++n_item) {
-        KV4_LANE_WAIT(kItemFull + (n_item & 1u), (n_item >> 1) & 1u, kWaitFullTimeout)
+        KV4_WAIT(kItemFull + (n_item & 1u), (n_item >> 1) & 1u, kWaitFullTimeout)
         const int valid = slots[n_item & 1u].valid, n_tiles = slots[n_item & 1u].n_tiles;
         __syncwarp();
         if (!valid) break;
         if (lane == 0) mbar_arrive(&bars[kItemEmpty + (n_item & 1u)]);
-        KV4_LANE_WAIT(kQFull, n_item & 1u, kWaitFullTimeout)
+        KV4_WAIT(kQFull, n_item & 1u, kWaitFullTimeout)
         if (n_tiles == 0) {              // nothing to multiply, but the Q tile must be released
           if (lane == 0) mbar_arrive(&bars[kQEmpty]);
           continue;
         }
         bool dead = false;
         uint32_t slot_k = seq % kSlots;
-        KV4_LANE_WAIT(kKVFull + slot_k, (seq / kSlots) & 1u, kWaitFullTimeout)
+        KV4_WAIT(kKVFull + slot_k, (seq / kSlots) & 1u, kWaitFullTimeout)
         ++seq;
         tcgen05_fence_after();
         issue_qk(0, slot_k);
@@ -453,17 +460,17 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
           const bool more = j + 1 < n_tiles;
           const uint32_t slot_v = seq % kSlots;
           dead = true;
-          KV4_LANE_WAIT(kKVFull + slot_v, (seq / kSlots) & 1u, kWaitMmaTimeout)
+          KV4_LANE_WAIT(kKVFull + slot_v, (seq / kSlots) & 1u)
           ++seq;
           uint32_t slot_k2 = 0;
           if (more) {
             slot_k2 = seq % kSlots;
-            KV4_LANE_WAIT(kKVFull + slot_k2, (seq / kSlots) & 1u, kWaitMmaTimeout)
+            KV4_LANE_WAIT(kKVFull + slot_k2, (seq / kSlots) & 1u)
             ++seq;
           }
           int w = 0;
           for (; w < 2; ++w) {
-            KV4_LANE_WAIT(kPFull + w, cp[w] & 1u, kWaitMmaTimeout)
+            KV4_LANE_WAIT(kPFull + w, cp[w] & 1u)
             ++cp[w];
             tcgen05_fence_after();
             const UmmaDesc vd = v_desc0 + (uint32_t)((slot_v * kTileBytes) >> 4);
@@ -471,7 +478,7 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
             for (int ks = 0; ks < 4; ++ks)
               umma_ts_f16_lead(lead, tmem_base + 2 * kBN + w * kHD, tmem_base + w * kBN + ks * 8,
                                vd + (uint32_t)((ks * 2048) >> 4), kIdescPV, (j > 0) | (ks > 0));
-            KV4_LANE_WAIT(kPLast + w, (cp[w] - 1) & 1u, kWaitMmaTimeout)
+            KV4_LANE_WAIT(kPLast + w, (cp[w] - 1) & 1u)
             tcgen05_fence_after();
 #pragma unroll
             for (int ks = 4; ks < 8; ++ks)
@@ -486,7 +493,10 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
           if (more) umma_commit_lead(lead, &bars[kKVEmpty + slot_k2]);
           if (j + 2 == n_tiles) umma_commit_lead(lead, &bars[kQEmpty]);
         }
-        if (dead) break;
+        if (__any_sync(0xffffffffu, dead)) {
+          KV4_REPORT(kWaitMmaTimeout)
+          break;
+        }
       }
       __syncwarp();
     }
