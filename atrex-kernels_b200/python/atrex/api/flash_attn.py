@@ -49,6 +49,7 @@ _HEAD_DIMS = (128, 256)
 # E4M3 runs on the single-tile tcgen05 kernel (the mma.sync kernel is BF16 only, and it is the one with softcap).
 _FP8_ROUTE_BUILT = True
 _MAX_SPLITS = 256
+_WIDEST_WINDOW = 2**30   # a side beyond it is as good as unbounded; the kernels' 32-bit positions may be added to it
 
 # (argument, value that means "not used", message) for vLLM arguments that no
 # ATREX target consumes (python/atrex/api/flash_attn.py:109-151).
@@ -287,7 +288,7 @@ def _validate_flash_attn_call(call):
     window = (-1, -1) if call["window_size"] is None else tuple(call["window_size"])
     if len(window) != 2:
         raise ValueError("window_size must contain two values")
-    window = tuple(-1 if w is None else int(w) for w in window)
+    window = tuple(-1 if w is None else max(-1, min(int(w), _WIDEST_WINDOW)) for w in window)
     softcap, logits_soft_cap = call["softcap"], call["logits_soft_cap"]
     if logits_soft_cap is not None:
         if softcap not in (0, 0.0, logits_soft_cap):

@@ -80,6 +80,13 @@ struct alignas(64) FwdParams {
   int8_t v_perm[3];
 };
 
+// One side of a window as the kernels take it: -1 = unbounded, and small enough that a position plus or minus it fits 32
+// bits (2^31 - 1, say, would wrap to a window that shows nothing).
+inline int32_t window_of(int32_t window) {
+  constexpr int32_t kWidest = 1 << 30;
+  return window < 0 ? -1 : window < kWidest ? window : kWidest;
+}
+
 // KV length and the first K row (packed K/V) of request b.  Lengths are clamped to what the caller's buffers can
 // hold, so a stale or corrupt length (a graph replayed after its metadata was overwritten) never becomes an
 // out-of-range page-table or row index: paged, at most the table row's width in keys; packed, at most the rows

@@ -411,8 +411,8 @@ int atrex_kv4_sm100_forward(const atrex_kv4_sm100_params* pp, void* workspace, u
   f.num_q_heads = p->num_q_heads; f.num_kv_heads = p->num_kv_heads;
   f.group = p->num_q_heads / p->num_kv_heads;
   f.causal = p->causal ? 1 : 0;
-  f.window_left = p->window_left < 0 ? -1 : p->window_left;
-  f.window_right = p->causal ? 0 : (p->window_right < 0 ? -1 : p->window_right);
+  f.window_left = window_of(p->window_left);
+  f.window_right = p->causal ? 0 : window_of(p->window_right);
   f.num_splits = r.splits;
   const int64_t cap = (int64_t)p->max_pages_per_seq * p->page_size;
   f.kv_cap = (int32_t)(cap > 0x7FFFFFFFll ? 0x7FFFFFFFll : cap);

@@ -562,8 +562,8 @@ int atrex_fa_sm100_forward(const atrex_fa_sm100_params* p, void* workspace, uint
   f.num_q_heads = p->num_q_heads; f.num_kv_heads = p->num_kv_heads;
   f.group = p->num_q_heads / p->num_kv_heads;
   f.causal = p->causal ? 1 : 0;
-  f.window_left = p->window_left < 0 ? -1 : p->window_left;
-  f.window_right = p->causal ? 0 : (p->window_right < 0 ? -1 : p->window_right);
+  f.window_left = window_of(p->window_left);
+  f.window_right = p->causal ? 0 : window_of(p->window_right);
   f.num_splits = r.splits;
   f.num_row_tiles = r.num_row_tiles;
   {

@@ -839,3 +839,13 @@ def test_tail_split_of_the_last_round():
     del poison
     T.check(case, requests=[0, 40, 73, 74, 75, 79], window_size=(511, 0), s_aux=sink)
     T.check(case, requests=[0, 73, 74, 79])
+
+
+@pytest.mark.parametrize("window,same", [((2**31 - 1, 2**31 - 1), (-1, -1)), ((2**40, 7), (-1, 7)), ((30, 2**31 - 1), (30, -1))])
+def test_very_wide_windows(window, same, route):
+    """A side as wide as an int32 or wider shows what an unbounded one does."""
+    case = T.make_case(64, [4, 1, 130, 70], [700, 300, 260, 30], hq=8, hkv=2, std=0.6)
+    got = T.run(case, causal=False, window_size=window)
+    want = T.run(case, causal=False, window_size=same)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    T.check(case, causal=False, window_size=same)

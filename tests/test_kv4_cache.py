@@ -87,6 +87,24 @@ def test_calls_that_are_served(as_b200):
                                                 window_size=(100, 0), return_softmax_lse=True, num_splits=3)
 
 
+@pytest.mark.parametrize("given,taken", [
+    ((5, None), (5, -1)), ((2**31 - 1, 0), (2**30, 0)), ((2**32 + 5, 2**63), (2**30, 2**30)), ((-2**33 + 3, -2), (-1, -1))])
+def test_windows_wider_than_32_bits(as_b200, given, taken):
+    """They neither wrap to a small window nor to one that shows nothing."""
+    seen = {}
+
+    def validate(call, real=as_b200._validate_flash_attn_call):
+        seen["result"] = real(call)
+        raise NotImplementedError("stop here")
+
+    as_b200._validate_flash_attn_call, real = validate, as_b200._validate_flash_attn_call
+    try:
+        assert not atrex.can_use_flash_attn_varlen_func(**dict(_call(), causal=False), window_size=given)
+    finally:
+        as_b200._validate_flash_attn_call = real
+    assert seen["result"][1] == taken
+
+
 BAD = [
     (dict(k_block_scale=None), ValueError, "block scales"),
     (dict(v_block_scale=None), ValueError, "block scales"),
@@ -855,3 +873,21 @@ def test_write_refuses_outs_that_overlap_its_inputs():
     kv_cache.write_kv_cache(rows, rows, k, v, slots, key_block_scale=ks, value_block_scale=vs, key_out=other)
     want = torch.from_numpy(kv4_oracle.quantise(rows.float().cpu().numpy())[2]).float().bfloat16()
     assert torch.equal(other.cpu(), want) and torch.equal(store, before) and torch.equal(k, v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 3, 6], [700, 2, 260]), ([160, 90], [400, 30])])
+@pytest.mark.parametrize("window,same", [((2**31 - 1, 2**31 - 1), (-1, -1)), ((2**40, 5), (-1, 5)), ((33, 2**31 - 1), (33, -1))])
+def test_very_wide_windows(q_lens, kv_lens, window, same, route):
+    """As wide as an int32 or wider: what an unbounded side shows.  Through the C block, too, which is given as it is."""
+    c = make_case(q_lens, kv_lens, 8, 2, 128, 64, seed=3)
+    args = gpu_args(c, causal=False)
+    out, lse = atrex.flash_attn_varlen_func(**args, window_size=window)
+    check(c, out, lse, False, same)
+    direct = {k: args[k] for k in ("q", "k", "v", "k_block_scale", "v_block_scale", "cu_seqlens_q", "seqused_k", "max_seqlen_q",
+                                   "max_seqlen_k")}
+    left, right = (min(w, 2**31 - 1) for w in window)
+    out, lse = kv4.forward(**direct, page_table=args["block_table"], softmax_scale=128 ** -0.5, causal=False, window_left=left,
+                           window_right=right, sink=None, out=None, return_lse=True, k_descale=None, v_descale=None,
+                           num_splits=0)
+    check(c, out, lse, False, same)
