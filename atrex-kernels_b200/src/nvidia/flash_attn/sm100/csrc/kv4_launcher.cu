@@ -209,23 +209,24 @@ int resolve(const atrex_kv4_sm100_params* pp, int sm_count, Resolved* r) {
   int64_t splits = r->kernel == kDouble ? 1 : p->num_splits;
   if (splits == 0 && prefill) {
     // Items walk the SMs in rounds; an item costs about four tiles besides its own (Q rows, first scores, epilogue).
-    // A split call pays for its partial results: the combine kernel as much again and about a tile per split (it reads
-    // them one after the other), and their bytes, of which 4 MB written and read take a tile's 1.3 us.  `items` is an
-    // upper bound when tiled and lengths vary, so only a gain of more than a sixteenth counts; beyond four rounds nothing
-    // is split, nor into more than 256 MB of partial results.  Microseconds by splits, head_dim 256 (requests, heads,
-    // query tokens, longest context):
-    //   15, 64 / 4, 1 .. 27, 12 406: 1: 242, 3: 160, 5: 165, 7: 169;  1, 64 / 4, 5, window 4 129: 8: 21, 16: 30, 34: 39
-    //   16, 24 / 2, 1 .. 96, 8 192: 1: 185, 2: 160, 4: 157, 5: 171;   59, 12 / 1, 10 .. 27, 2 027: 1: 65, 2: 80
-    //   1, 64 / 8, 512, 16 384: 1: 680, 2: 734, 5: 751;   3, 32 / 8, 900 .. 1 060, 12 974: 1: 1 073, 2: 1 144, 3: 1 171
+    // Splitting costs eight tiles (the combine kernel, the start of smaller items) and the partial results, of which
+    // 1.5 MB written and read take a tile's 1.3 us.  An unsplit call counts an eighth more, because it waits for its
+    // longest item and lengths vary; beyond three rounds nothing is split, nor into more than 256 MB.  The constants are
+    // those with the least loss over 27 shapes measured with 1 .. 48 splits, 3 % on average, 18 % at most.  Microseconds by
+    // splits, the rule's choice in brackets (requests, heads of D, query tokens, contexts):
+    //   1, 64 / 4 of 128, 5, 16 384:  1: 226, 4: 68, 16: 29, [32: 25], 48: 37;    8, same, 8 192:  1: 120, [4: 43], 8: 48
+    //   30, 64 / 4 of 128, 8, 500 .. 30 000:  1: 379, 4: 281, [6: 300];   all 20 000:  [1: 280], 2: 303, 6: 287
+    //   40, 64 / 8 of 128, 10, 4 000 .. 16 000:  1: 424, [3: 373];   20, same, 9 .. 15, 1 000 .. 9 000:  1: 195, [3: 128], 5: 178
+    //   16, 24 / 2 of 256, 1 .. 96, 97 .. 8 192:  1: 185, [3: 158], 6: 184;   90 .. 96, 8 192:  1: 361, [2: 419], 4: 476
+    //   1, 64 / 8 of 256, 512, 16 384:  1: 680, [2: 731], 5: 748;   3, 32 / 8, ~1 000, 5 000 .. 12 974:  [1: 1 065], 3: 1 168
     const int64_t part = 4 * (int64_t)p->total_q * p->num_q_heads * (p->head_dim + 1);     // bytes of a split's results
-    int64_t unsplit = 0, best = 0;
+    int64_t best = 0;                                                                      // in eighths of a tile
     splits = 1;
-    for (int64_t s = 1; s <= most && s <= 64 && (s == 1 || items <= 4 * (int64_t)sm_count); ++s) {
-      int64_t cost = ((items * s + sm_count - 1) / sm_count) * ((most + s - 1) / s + 4);
-      if (s > 1 && s * part > (256 << 20)) break;
-      if (s > 1) cost += 4 + s + s * part / (4 << 20);
-      if (s == 1) unsplit = best = cost;
-      if (cost < best && cost * 16 < unsplit * 15) {
+    for (int64_t s = 1; s <= most && s <= 64; ++s) {
+      if (s > 1 && (items > 3 * (int64_t)sm_count || s * part > (256 << 20))) break;
+      const int64_t tiles_long = ((items * s + sm_count - 1) / sm_count) * ((most + s - 1) / s + 4);
+      const int64_t cost = s == 1 ? 9 * tiles_long : 8 * tiles_long + 64 + s * part / (192 << 10);
+      if (s == 1 || cost < best) {
         best = cost;
         splits = s;
       }
