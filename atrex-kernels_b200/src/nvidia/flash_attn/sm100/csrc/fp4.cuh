@@ -76,11 +76,13 @@ __device__ __forceinline__ void row_power(uint32_t top, float& up, float& down) 
   down = e == 254 ? 0x1p-127f : __int_as_float((254 - e) << 23);
 }
 // Score factor of a row: positive (a negative scale goes into the sign of Q) and never zero, so that a masked score
-// stays -inf when it is multiplied by it.  A NaN stays, and makes the scores of the row NaN; a row that sees no key is
-// empty whatever its scale.
-__device__ __forceinline__ float score_factor(float scale, bool sees_keys) {
+// stays -inf when it is multiplied by it.  A NaN stays, and makes the scores of the row NaN, unless the row sees no key: it
+// is empty whatever its scale.  `sees_keys` is asked about NaN scales only (the decode kernel pays 1 - 2 % for asking always).
+template <typename SeesKeys>
+__device__ __forceinline__ float score_factor(float scale, const SeesKeys& sees_keys) {
+  if (scale != scale && !sees_keys()) scale = 0.f;
   const float a = fabsf(scale);
-  return a < 1.2e-38f || !sees_keys ? 1.2e-38f : a;
+  return a < 1.2e-38f ? 1.2e-38f : a;
 }
 
 }  // namespace atrex_sm100

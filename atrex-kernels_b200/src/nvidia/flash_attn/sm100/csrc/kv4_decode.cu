@@ -299,9 +299,11 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 2 ? 3 : 1) atrex_sm100_kv4_
         }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        int lo, hi;
-        row_keys(nb * 8 + 2 * t + i, lo, hi);
-        factor[nb][i] = score_factor(__shfl_sync(0xffffffffu, down, 8 * t + 4 * i) * scale_log2, lo < hi);
+        factor[nb][i] = score_factor(__shfl_sync(0xffffffffu, down, 8 * t + 4 * i) * scale_log2, [&] {
+          int lo, hi;
+          row_keys(nb * 8 + 2 * t + i, lo, hi);
+          return lo < hi;
+        });
       }
     }
   }

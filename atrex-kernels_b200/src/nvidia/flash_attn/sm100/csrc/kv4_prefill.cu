@@ -525,7 +525,7 @@ atrex_sm100_kv4_prefill_kernel(const __grid_constant__ Kv4Params pp) {
       const int qi = min((it.row0 + r) / p.group, max(it.q_len - 1, 0));
       const int vis_hi = p.window_right >= 0 ? min(it.kv_len, right_bound(p, qi + it.off)) : it.kv_len;
       const int vis_lo = p.window_left >= 0 ? max(0, qi + it.off - p.window_left) : 0;
-      scale_log2 = score_factor(scale_log2, vis_lo < vis_hi);
+      scale_log2 = score_factor(scale_log2, [&] { return vis_lo < vis_hi; });
       const int sqi_lo = it.row0 / p.group;
       const int sqi_hi = min(it.q_len - 1, (it.row0 + kRows - 1) / p.group);
       const int full_lo = p.window_left >= 0 ? max(0, sqi_hi + it.off - p.window_left) : 0;

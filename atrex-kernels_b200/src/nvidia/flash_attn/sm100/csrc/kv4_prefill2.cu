@@ -194,7 +194,7 @@ __device__ __forceinline__ void widen_row(const uint8_t* stage, uint8_t* tile, i
     atomicExch(abort_flag, 1);                        \
   }
 // A warp goes on or leaves its loop as one: TMEM accesses and warp barriers behind a wait need all of its lanes.  The tile
-// loops of issuer and producers hold neither, because a vote there costs (chunk case, us: 1 830; at every wait 1 900, in
+// loops of issuer and producers hold neither, because a vote there costs (chunk case, us: 1 835; at every wait 1 900, in
 // place of the producers' barrier behind a stage 1 885): their lanes give up one by one and the warp votes once an item.
 #define KV4_WAIT(bar_index, parity, code)                                          \
   if (!__all_sync(0xffffffffu, mbar_wait(&bars[bar_index], (parity)))) {           \
@@ -516,6 +516,7 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
       if (!it.valid) break;
       const int sub_row0 = it.row0 + w * kBM;
       const int n_tiles = it.n_tiles, tile_lo = it.tile_lo;
+      float scale_log2 = it.scale_log2 * row_factor[(n_item & 1u) * kRowsPerItem + w * kBM + r];
       int vis_lo, vis_hi, full_lo, full_hi;
       {
         const int q_last = max(it.q_len - 1, 0), off = it.off, kv_len = it.kv_len;
@@ -526,8 +527,7 @@ atrex_sm100_kv4_prefill2_kernel(const __grid_constant__ Kv4Params pp) {
         full_lo = p.window_left >= 0 ? max(0, sqi_hi + off - p.window_left) : 0;
         full_hi = p.window_right >= 0 ? min(kv_len, right_bound(p, sqi_lo + off)) : kv_len;
       }
-      const float scale_log2 =
-          score_factor(it.scale_log2 * row_factor[(n_item & 1u) * kRowsPerItem + w * kBM + r], vis_lo < vis_hi);
+      scale_log2 = score_factor(scale_log2, [&] { return vis_lo < vis_hi; });
       bool dead = false;
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = 0; j < n_tiles; ++j) {
