@@ -185,6 +185,12 @@ int resolve(const atrex_kv4_sm100_params* pp, int sm_count, Resolved* r) {
   const int64_t packed = (int64_t)p->max_seqlen_q * group;      // query rows per (request, KV head), at most
   const bool prefill = p->route == ATREX_FA_ROUTE_UMMA || (p->route == ATREX_FA_ROUTE_AUTO &&
                         packed > max_decode_rows((int64_t)p->batch * p->num_kv_heads, p->head_dim, sm_count));
+  // Two-tile or single-tile, unsplit or by the split rule below (us, head_dim 128; requests, heads, query tokens, contexts):
+  //   items that fill the SMs: 4, 64 / 8, 512 .. 2 048, 4 096 .. 16 384: 1 823 / 2 626;  1, 32 / 8, 2 048, 16 384: 542 / 863;
+  //     64, 64 / 4, 9, 2 000 .. 8 000: 248 / 309;  16, 32 / 8, 200 .. 1 000, 1 000 .. 4 000: 625 / 573;  64 of 60 .. 200: 148 / 142
+  //   items that leave SMs idle, where the two-tile kernel, which is never split, is the wrong choice: 1 over 16 384 keys,
+  //     8 / 1 heads: 32 .. 128 tokens 263 / 41, 512: 263 / 78, 2 048: 263 / 232;  32 / 8 heads: 128: 265 / 97, 512: 264 / 235
+  // A caller of one such prompt gets the second figure with num_splits (2 or more).
   r->kernel = !prefill ? kDecode
               : p->head_dim == 128 && packed > kv4_prefill_rows() && p->num_splits <= 1 ? kDouble : kSingle;
   r->rows = r->kernel == kDouble ? kv4_prefill2_rows()

@@ -15,10 +15,11 @@
 //   warps 12-15  widening: 32 rows each of every tile, from the staging ring into the FP16 operand ring; at the start of
 //                an item its Q rows, 64 each (a row is scaled by a power of two that joins its score factor)
 //
-// Measured: 4 chunks of 512 .. 2 048 tokens over contexts of 4 096 .. 16 384, 64 / 8 heads of 128: 1.81 ms = 960 TFLOP/s
-// (the single-tile kernel: 3.71 ms).  What bounds it: a subtile's chain of softmax (~1 900 cycles per 128 keys, waiting for
-// its own instructions, their fetch included: polynomial exponentials, which free the special-function units, made it
-// 1 930 -> 2 270 us) and the two products behind it (512 each), of which the other subtile covers what it can.
+// Measured: 4 chunks of 512 .. 2 048 tokens over contexts of 4 096 .. 16 384, 64 / 8 heads of 128: 1.83 ms = 950 TFLOP/s
+// (the single-tile kernel: 2.63 ms; where it wins, the launcher says).  What bounds it: a subtile's chain of softmax
+// (~1 900 cycles per 128 keys, waiting for its own instructions, their fetch included: polynomial exponentials, which free
+// the special-function units, made it 1 930 -> 2 270 us) and the two products behind it (512 each), of which the other
+// subtile covers what it can.
 //
 // Both products are FP16: E2M1 x E4M3 is exact there (fp4.cuh), P is stored as 2^7 p.  Every wait is bounded; on expiry
 // the CTA records a code, drains its copies, frees TMEM and returns.

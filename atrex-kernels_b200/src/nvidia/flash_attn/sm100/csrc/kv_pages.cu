@@ -5,9 +5,10 @@
 // copied byte is read and written once, bound by HBM.  Destinations are pages that were free before the call and
 // sources are pages that were held, so no page is both and the copies need no order.
 //
-// Small pools take one kernel whose CTAs each make the whole plan for themselves.  Larger ones: reassign: one CTA makes the list of copies (a batch has few rows; the free pages it needs are found by scanning the
-// counts from the front until there are enough) while the others copy the counts; a second kernel writes tables and
-// counts and copies the tokens.  compact: per-chunk counts, then lists, then tables, counts and copies.
+// Small pools take one kernel whose CTAs each make the whole plan for themselves.  In larger ones, reassign: one CTA makes
+// the list of copies (a batch has few rows; the free pages it needs are found by scanning the counts from the front until
+// there are enough) while the others copy the counts; a second kernel writes tables and counts and copies the tokens.
+// compact: per-chunk counts, then lists, then tables, counts and copies.
 #include <algorithm>
 #include <atomic>
 #include <cstring>

@@ -50,7 +50,8 @@ def forward(*, q, k, v, cu_seqlens_q, cu_seqlens_k, seqused_k, max_seqlen_q, max
             return_lse, q_descale, k_descale, v_descale, num_splits, route=None, cp_world_size=1, cp_rank=0,
             cp_tot_seqused_k=None, layout_token=None):
     """``layout_token``: optional hashable value that determines every argument except tensor addresses (the
-    public API passes its call signature); it then serves as the layout key instead of one computed here."""
+    public API passes a number that stands for the call's signature); it then serves as the layout key instead of one
+    computed here."""
     if route is None:
         route = DEFAULT_ROUTE
     if out is None:
