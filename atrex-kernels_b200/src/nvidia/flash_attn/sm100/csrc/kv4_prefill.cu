@@ -16,11 +16,12 @@
 //
 // Measured: 64 requests x 4 query tokens, window 4 095, 64 / 4 heads of 128: 109 us (23 for the bytes); 16 requests of
 // 1 .. 96 query tokens, 24 / 2 heads of 256, contexts of 97 .. 8 192: 158 us (33).  A tile of 128 rows by 128 keys takes
-// ~2 550 cycles there (in long prompts 3 400, where the two-tile kernel takes 2 350), and three chains in it are about equally long: widening (two units of
-// ~1 170 cycles on four warps), the softmax threads (half of a row each: load, exchange, exponentials, hand-over) and at
-// head_dim 256 the tensor pipe (20 MMAs, ~88 cycles each).  Shortening one alone gained nothing: eight widening warps beside
-// four softmax warps 109 -> 120 and 158 -> 164 us; pairs of warps per row piece 109 -> 124; the next unit's codes in
-// registers early 109 -> 112; polynomial exponentials 109 -> 117; 128-key tiles at head_dim 256 155 -> 179.
+// ~2 550 cycles there (in long prompts 3 400, where the two-tile kernel takes 2 350), and three chains in it are about
+// equally long: widening (two units of ~1 170 cycles on four warps), the softmax threads (half of a row each: load,
+// exchange, exponentials, hand-over) and at head_dim 256 the tensor pipe (20 MMAs, ~88 cycles each).  Shortening one alone
+// gained nothing: eight widening warps beside four softmax warps 109 -> 120 and 158 -> 164 us; pairs of warps per row piece
+// 109 -> 124; the next unit's codes in registers early 109 -> 112; polynomial exponentials 109 -> 117; 128-key tiles at
+// head_dim 256 155 -> 179.
 //
 // Every wait is bounded; on expiry the CTA records a code, drains its copies, frees TMEM and returns.
 #define ATREX_MBAR_SPIN_INLINE   // setmaxnreg: no calls with their own register ABI
