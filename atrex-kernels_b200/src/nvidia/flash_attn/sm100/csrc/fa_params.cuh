@@ -87,6 +87,14 @@ inline int32_t window_of(int32_t window) {
   return window < 0 ? -1 : window < kWidest ? window : kWidest;
 }
 
+// Most keys that a page-table row can name.  Ends 2^16 short of 2^31: the kernels' 32-bit key indices run on past the last
+// key, by a ring of tiles and (decode over a 4-bit cache) the 32 tiles whose pages are fetched together, 4 352 keys.
+inline int32_t kv_cap_of(int32_t pages, int32_t page_size) {
+  constexpr int64_t kMost = (1ll << 31) - (1ll << 16);
+  const int64_t keys = (int64_t)pages * page_size;
+  return (int32_t)(keys < kMost ? keys : kMost);
+}
+
 // KV length and the first K row (packed K/V) of request b.  Lengths are clamped to what the caller's buffers can
 // hold, so a stale or corrupt length (a graph replayed after its metadata was overwritten) never becomes an
 // out-of-range page-table or row index: paged, at most the table row's width in keys; packed, at most the rows

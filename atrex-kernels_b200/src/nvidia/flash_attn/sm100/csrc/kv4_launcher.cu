@@ -190,7 +190,7 @@ int resolve(const atrex_kv4_sm100_params* pp, int sm_count, Resolved* r) {
   //     64, 64 / 4, 9, 2 000 .. 8 000: 248 / 309;  16, 32 / 8, 200 .. 1 000, 1 000 .. 4 000: 625 / 573;  64 of 60 .. 200: 148 / 142
   //   items that leave SMs idle, where the two-tile kernel, which is never split, is the wrong choice: 1 over 16 384 keys,
   //     8 / 1 heads: 32 .. 128 tokens 263 / 41, 512: 263 / 78, 2 048: 263 / 232;  32 / 8 heads: 128: 265 / 97, 512: 264 / 235
-  // A caller of one such prompt gets the second figure with num_splits (2 or more).
+  // A call with num_splits of 2 or more takes the single-tile kernel: with one that fills the SMs, about the second figure.
   r->kernel = !prefill ? kDecode
               : p->head_dim == 128 && packed > kv4_prefill_rows() && p->num_splits <= 1 ? kDouble : kSingle;
   r->rows = r->kernel == kDouble ? kv4_prefill2_rows()

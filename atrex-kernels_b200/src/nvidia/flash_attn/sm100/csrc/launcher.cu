@@ -566,10 +566,7 @@ int atrex_fa_sm100_forward(const atrex_fa_sm100_params* p, void* workspace, uint
   f.window_right = p->causal ? 0 : window_of(p->window_right);
   f.num_splits = r.splits;
   f.num_row_tiles = r.num_row_tiles;
-  {
-    const int64_t cap = paged ? (int64_t)p->max_pages_per_seq * p->page_size : 0;
-    f.kv_cap = (int32_t)(cap > 0x7FFFFFFFll ? 0x7FFFFFFFll : cap);
-  }
+  f.kv_cap = paged ? kv_cap_of(p->max_pages_per_seq, p->page_size) : 0;
   f.cp_world_size = p->cp_world_size > 1 ? p->cp_world_size : 1;
   f.cp_rank = p->cp_world_size > 1 ? p->cp_rank : 0;
   f.cp_tot_seqused_k = p->cp_world_size > 1 ? p->cp_tot_seqused_k : nullptr;
